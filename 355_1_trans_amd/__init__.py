@@ -276,6 +276,13 @@ def _record(stream, *tensors):
             t.record_stream(stream)
 
 
+def _int32(name, *values):
+    """Sizes and pitches that the library takes as 32-bit integers; ctypes
+    would cut a larger one without an error."""
+    if any(v > 0x7FFFFFFF for v in values):
+        raise ValueError(f"{name}: sizes and row pitches must be below 2**31")
+
+
 def _require_gpu(*tensors):
     dev = tensors[0].device
     if not tensors[0].is_cuda:

@@ -3,15 +3,15 @@ linear layers (bias, activation, residual) and gated feed-forward blocks on
 MXFP8 / MXFP4 operands, and their gradients.
 
 Calls launch on the current stream and record every tensor on it; there is no
-CPU fallback.  Gradients take the tensors that the forward call used and
+CPU fallback.  Sizes and row pitches (in elements) are below 2**31.  Gradients take the tensors that the forward call used and
 returned; nothing is kept between calls.
 """
 import ctypes
 
 import torch
 
-from . import (_WORKSPACES, Epilogue, Kargs, LayerGrad, _check, _out, _out_code, _record, _require_gpu, _stream,
-               _workspace_of, _ws_tensor, fast, lib)
+from . import (_WORKSPACES, Epilogue, Kargs, LayerGrad, _check, _int32, _out, _out_code, _record, _require_gpu,
+               _stream, _workspace_of, _ws_tensor, fast, lib)
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -31,7 +31,9 @@ def _rows(t, name, like=None):
         raise ValueError(f"{name} must have the shape and dtype of the tensor beside it")
     if t.shape[1] == 0 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise ValueError(f"{name} needs at least one column and contiguous rows that do not overlap")
-    return _TYPES[t.dtype], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    _int32(name, *t.shape, ld)
+    return _TYPES[t.dtype], ld
 
 
 def _vectors(n, *pairs):
@@ -128,6 +130,7 @@ def _mx_operands(A, B, A_scale, B_scale, fp4):
         raise ValueError(f"requires matching K with K % {step} == 0 and at least one row of B")
     if A_scale.shape != (m, k // 32) or B_scale.shape != (n, k // 32):
         raise ValueError("requires A_scale [M,K/32] and B_scale [N,K/32]")
+    _int32("A, B", m, n, k)
     kg = k // 32
     args = Kargs(A.data_ptr(), B.data_ptr(), None, m, n, k, 1, kb, kb, 0, 0, 0, 0, A_scale.data_ptr(),
                  B_scale.data_ptr(), kg, kg, 0, 0)
@@ -271,6 +274,7 @@ def _backward(dy, x, w, pre, features, activation, bias_grad, workspace):
     (m, k), n = x.shape, w.shape[0]
     if k == 0 or k % 8 or n == 0:
         raise ValueError("requires K % 8 == 0, at least one column and one row of w")
+    _int32("x, w", m, n, k)
     act = _activation(activation)
     if pre is None and (features or act):
         raise ValueError("pre (the forward call's save_pre) is needed")
