@@ -376,6 +376,7 @@ def gemm_a8w8_mxfp8(A, B, A_scale, B_scale, dtype=torch.bfloat16, out=None, work
     for t in (A, B, A_scale, B_scale):
         if not t.is_contiguous():
             raise ValueError("A, B and scales must be contiguous")
+    _int32("A, B", m, n, k)
     out = _out(out, (m, n), dtype, dev)
     args = Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, k, k, n, m * k, n * k, m * n,
                  A_scale.data_ptr(), B_scale.data_ptr(), k // 32, k // 32, m * (k // 32), n * (k // 32))
@@ -406,6 +407,7 @@ def gemm_a4w4_mxfp4(A, B, A_scale, B_scale, dtype=torch.bfloat16, out=None, work
     for t in (A, B, A_scale, B_scale):
         if not t.is_contiguous():
             raise ValueError("A, B and scales must be contiguous")
+    _int32("A, B", m, n, k)
     out = _out(out, (m, n), dtype, dev)
     args = Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, kb, kb, n, m * kb, n * kb, m * n,
                  A_scale.data_ptr(), B_scale.data_ptr(), k // 32, k // 32, m * (k // 32), n * (k // 32))
@@ -469,6 +471,7 @@ def gemm_a4w4(A, B, A_scale, B_scale, out=None, bias=None, alpha=1.0, beta=0.0, 
         raise ValueError("A and B must be contiguous")
     sfa = _shuffled_scale(A_scale, m, k // 32, "A_scale")
     sfb = _shuffled_scale(B_scale, n, k // 32, "B_scale")
+    _int32("A, B", m, n, k)
     out = _out(out, (m, n), dtype, dev)
     args = Mxfp4Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, kb, kb, n, m * kb, n * kb, m * n,
                       A_scale.data_ptr(), B_scale.data_ptr(), sfa, sfb, A_scale.numel(), B_scale.numel(),
@@ -509,6 +512,7 @@ def gemm_a8w8_bpreshuffle(A, B_kpanel, A_scale, B_scale, dtype=torch.bfloat16, o
     if not (A.is_contiguous() and B_kpanel.is_contiguous() and B_scale.is_contiguous()):
         raise ValueError("A, B_kpanel and B_scale must be contiguous")
     stride_sfa = _sfa_stride(A_scale, m)
+    _int32("A, B", m, n, k)
     out = _out(out, (m, n), dtype, dev)
     args = Kargs(A.data_ptr(), B_kpanel.data_ptr(), out.data_ptr(), m, n, k, 1, k, 128, n, m * k, n * k, m * n,
                  A_scale.data_ptr(), B_scale.data_ptr(), stride_sfa, kg, m * kg, B_scale.shape[0] * kg)
@@ -542,6 +546,7 @@ def ldsbypass_pack_b(B):
     if B.dim() != 2 or B.element_size() != 1:
         raise ValueError("B must be a 2-D [N, K] tensor of 1-byte elements")
     n, k = B.shape
+    _int32("B", n, k)
     nbytes = ldsbypass_b_bytes(n, k)
     if nbytes == 0:
         raise ValueError("requires N >= 1 and K % 128 == 0")
@@ -561,6 +566,7 @@ def ldsbypass_repack(B_kpanel, out=None):
     if B_kpanel.dim() != 3 or B_kpanel.shape[2] != 128 or not B_kpanel.is_contiguous():
         raise ValueError("B_kpanel must be a contiguous [K/128, N, 128] tensor")
     k, n = B_kpanel.shape[0] * 128, B_kpanel.shape[1]
+    _int32("B_kpanel", n, k)
     out = _out(out, (ldsbypass_b_bytes(n, k),), torch.uint8, dev)
     args = LdsBypassKargs(None, B_kpanel.data_ptr(), out.data_ptr(), None, 0, n, k, 1, 0, 128, 0, 0, n * k, 0,
                           None, None, 0, 0, 0, 0, out.numel())
@@ -591,6 +597,7 @@ def gemm_a8w8_ldsbypass(A, B_pp, A_scale, B_scale, n, dtype=torch.bfloat16, out=
     if not (A.is_contiguous() and B_pp.is_contiguous() and B_scale.is_contiguous()):
         raise ValueError("A, B_pp and B_scale must be contiguous")
     stride_sfa = _sfa_stride(A_scale, m)
+    _int32("A, B", m, n, k)
     out = _out(out, (m, n), dtype, dev)
     args = LdsBypassKargs(A.data_ptr(), None, B_pp.data_ptr(), out.data_ptr(), m, n, k, 1, k, 128, n, m * k,
                           n * k, m * n, A_scale.data_ptr(), B_scale.data_ptr(), stride_sfa, kg, m * kg,
@@ -674,6 +681,7 @@ def _group_kargs(kind, A, B, A_scale, B_scale, out, n):
         if B.dim() != 2 or B.shape[1] != kb or A_scale.shape != (m, k // 32) or B_scale.shape != (B.shape[0], k // 32):
             raise ValueError(f"{kind}: A [M,{'K/2' if fp4 else 'K'}], B [N,...], scales [rows, K/32]")
         n = B.shape[0]
+        _int32("A, B", m, n, k)
         return Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, kb, kb, n, m * kb, n * kb, m * n,
                      A_scale.data_ptr(), B_scale.data_ptr(), k // 32, k // 32, m * (k // 32), n * (k // 32))
     k = A.shape[1]
@@ -686,6 +694,7 @@ def _group_kargs(kind, A, B, A_scale, B_scale, out, n):
         raise ValueError("ldsbypass: give N for each B'' (problems as (A, B'', A_scale, B_scale, N))")
     if A_scale.shape != (m, kg) or B_scale.shape != ((n + 127) // 128, kg) or not B_scale.is_contiguous():
         raise ValueError("block scales: A_scale fp32 [M,K/128], B_scale fp32 [ceil(N/128),K/128]")
+    _int32("A, B", m, n, k)
     sfa = _sfa_stride(A_scale, m)
     if kind == "bpreshuffle":
         return Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, k, 128, n, m * k, n * k, m * n,
@@ -768,6 +777,7 @@ def reference_gemm(kind, A, B, A_scale, B_scale):
         sfa, sfb = A_scale.stride(0), B_scale.stride(0)
     else:
         sfa, sfb = _sfa_stride(A_scale, m), B_scale.stride(0)
+    _int32("A, B", m, n, k)
     out = torch.empty((m, n), dtype=torch.float32, device=dev)
     args = Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, kb, kb, n, 0, 0, 0,
                  A_scale.data_ptr(), B_scale.data_ptr(), sfa, sfb, 0, 0)

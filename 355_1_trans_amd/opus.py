@@ -26,7 +26,7 @@ from pathlib import Path
 
 import torch
 
-from . import Kargs, _Address, _check, _out_code, _record, _require_gpu, _stream, lib, shuffle_b_kpanel
+from . import Kargs, _Address, _check, _int32, _out_code, _record, _require_gpu, _stream, lib, shuffle_b_kpanel
 
 CONFIGS = Path(__file__).resolve().parent / "configs"
 
@@ -121,6 +121,7 @@ def gemm_a8w8_bpreshuffle_opus(A, B, x_scale, w_scale, out_dtype=torch.bfloat16,
     for t in (A3, Bk, xs, ws_):
         if not t.is_contiguous():
             raise ValueError("A, B and the scales must be contiguous")
+    _int32("A, B", m, n, k)
     out = torch.empty((batch, m, n), dtype=out_dtype, device=dev)
     if kernelId is None:
         kernelId = lookup_tuned(_cu_num(dev), m, n, k, out_dtype) if batch == 1 else None
@@ -163,6 +164,7 @@ def gemm_a8w8_mxfp8_opus(A, B, x_scale, w_scale, out=None):
         if tuple(out.shape) not in shapes or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError("out must be a contiguous fp32 [batch, M, N] tensor ([M, N] only when batch is 1)")
     dev = _require_gpu(A, B, x_scale, w_scale) if out is None else _require_gpu(A, B, x_scale, w_scale, out)
+    _int32("A, B", m, n, k)
     if out is None:
         out = torch.empty((batch, m, n), dtype=torch.float32, device=dev)
     args = Kargs(A3.data_ptr(), B3.data_ptr(), out.data_ptr(), m, n, k, batch, k, k, n, m * k, n * k, m * n,
@@ -197,6 +199,7 @@ def _layout_gemm(layout, A, B, sfa, sfb, out):
         raise ValueError("sfb must be contiguous E8M0 bytes [N/128, K/128]")
     if not (A.is_contiguous() and B.is_contiguous() and out.is_contiguous()):
         raise ValueError("A, B and out must be contiguous")
+    _int32("A, B", m, n, k)
     kg = k // 128
     args = Kargs(A.data_ptr(), B.data_ptr(), out.data_ptr(), m, n, k, 1, m if a_t else k, n if b_n else k, n,
                  m * k, n * k, m * n, sfa.data_ptr(), sfb.data_ptr(), m, kg, m * kg, (n // 128) * kg)

@@ -24,7 +24,7 @@ import ctypes
 
 import torch
 
-from . import _check, _record, _require_gpu, _stream, fast, lib
+from . import _check, _int32, _record, _require_gpu, _stream, fast, lib
 
 IN_FP32, IN_BF16 = 0, 1
 
@@ -36,7 +36,9 @@ def _source(x, k_align):
     if x.stride(1) != 1 or x.stride(0) % 4 or x.shape[1] % k_align:
         raise ValueError(f"x needs contiguous rows, a row pitch that is a multiple of 4 elements and "
                          f"K % {k_align} == 0")
-    return (IN_FP32 if x.dtype == torch.float32 else IN_BF16), x.stride(0)
+    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]    # one row: any pitch
+    _int32("x", *x.shape, ld)
+    return (IN_FP32 if x.dtype == torch.float32 else IN_BF16), ld
 
 
 def _launch(x, fn_name, *args, keep=()):
@@ -145,6 +147,7 @@ def e8m0_shuffle(e):
     if e.dim() != 2 or e.element_size() != 1 or e.stride(1) != 1:
         raise ValueError("e must be a 2-D byte tensor with contiguous rows")
     rows, kg = e.shape
+    _int32("e", rows, kg, e.stride(0))
     out = torch.empty(e8m0_shuffle_bytes(rows, kg), dtype=torch.uint8, device=e.device)
     _launch(e, "qgemm_e8m0_shuffle_device", e.data_ptr(), out.data_ptr(), rows, kg, e.stride(0), keep=(out,))
     return out
@@ -156,6 +159,7 @@ def relayout_device(fn_name, B, out_bytes):
     if B.dim() != 2 or B.element_size() != 1 or B.stride(1) != 1 or B.stride(0) % 16:
         raise ValueError("B must be a 2-D byte tensor with contiguous rows and a pitch that is a multiple of 16")
     n, kb = B.shape
+    _int32("B", n, kb, B.stride(0))
     out = torch.empty(out_bytes, dtype=torch.uint8, device=B.device)
     _launch(B, fn_name, B.data_ptr(), out.data_ptr(), n, kb, B.stride(0), keep=(out,))
     return out
