@@ -19,7 +19,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <climits>
 
 #include "act_grad.hpp"
 #include "launch.hpp"
@@ -192,25 +191,30 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_kernel(const NormArgs 
 }
 
 // Rows past the registers: three passes over the row (the second and third
-// from cache), 1024 threads, one element at a time.
+// from cache), 1024 threads, one element at a time.  A thread's own sums, over
+// any number of elements, are in 64 bits.  n may be up to 2^31 - 1, which a
+// signed column counter would overflow on its way out of the loop.
 __global__ __launch_bounds__(1024) void norm_long_kernel(const NormArgs a) {
     __shared__ float lds[64];
     int half = 0;
+    const unsigned n = a.n;
     const float len = (float)a.n, inv = 1.0f / len;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long x0 = row * a.ldx, y0 = row * a.ldy;
-        float s[1] = {0.f};
-        for (int c = threadIdx.x; c < a.n; c += 1024) s[0] += load_f32(a.x, x0 + c, a.x_type);
+        double sum = 0.0;
+        for (unsigned c = threadIdx.x; c < n; c += 1024) sum += load_f32(a.x, x0 + c, a.x_type);
+        float s[1] = {(float)sum};
         row_sums<1024, 1>(s, lds, half);
         const float mean = mean_of(s[0], len, inv);
-        s[0] = 0.f;
-        for (int c = threadIdx.x; c < a.n; c += 1024) {
-            const float d = load_f32(a.x, x0 + c, a.x_type) - mean;
-            s[0] = __builtin_fmaf(d, d, s[0]);
+        sum = 0.0;
+        for (unsigned c = threadIdx.x; c < n; c += 1024) {
+            const double d = load_f32(a.x, x0 + c, a.x_type) - mean;
+            sum += d * d;
         }
+        s[0] = (float)sum;
         row_sums<1024, 1>(s, lds, half);
         const float rstd = rsqrtf(__builtin_fmaf(s[0], inv, a.eps));
-        for (int c = threadIdx.x; c < a.n; c += 1024) {
+        for (unsigned c = threadIdx.x; c < n; c += 1024) {
             const float w = a.weight ? load_f32(a.weight, c, a.w_type) : 1.f;
             const float b = a.bias ? load_f32(a.bias, c, a.w_type) : 0.f;
             const float y = __builtin_fmaf((load_f32(a.x, x0 + c, a.x_type) - mean) * rstd, w, b);
@@ -346,20 +350,22 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_grad_kernel(const Norm
 __global__ __launch_bounds__(1024) void norm_grad_long_kernel(const NormGradArgs a) {
     __shared__ float lds[64];
     int half = 0;
+    const unsigned n = a.n;
     const float inv = 1.0f / (float)a.n;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long x0 = row * a.ldx, g0 = row * a.lddy, d0 = row * a.lddx;
         const float mean = a.mean[row], rstd = a.rstd[row];
-        float s[2] = {0.f, 0.f};
-        for (int c = threadIdx.x; c < a.n; c += 1024) {
+        double sg = 0.0, sgx = 0.0;
+        for (unsigned c = threadIdx.x; c < n; c += 1024) {
             const float xh = (load_f32(a.x, x0 + c, a.x_type) - mean) * rstd;
             const float g = load_f32(a.dy, g0 + c, a.x_type) * (a.weight ? load_f32(a.weight, c, a.w_type) : 1.f);
-            s[0] += g;
-            s[1] = __builtin_fmaf(g, xh, s[1]);
+            sg += g;
+            sgx += (double)g * xh;
         }
+        float s[2] = {(float)sg, (float)sgx};
         row_sums<1024, 2>(s, lds, half);
         const float c0 = s[0] * inv, c1 = s[1] * inv;
-        for (int c = threadIdx.x; c < a.n; c += 1024) {
+        for (unsigned c = threadIdx.x; c < n; c += 1024) {
             const float xh = (load_f32(a.x, x0 + c, a.x_type) - mean) * rstd;
             const float g = load_f32(a.dy, g0 + c, a.x_type) * (a.weight ? load_f32(a.weight, c, a.w_type) : 1.f);
             const float d = rstd * __builtin_fmaf(-xh, c1, g - c0);
@@ -371,8 +377,8 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(const NormGradArgs
 // ... and partial rows of dw and db by columns: block y takes every
 // gridDim.y-th row.
 __global__ __launch_bounds__(256) void norm_grad_cols_kernel(const NormGradArgs a) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.n) return;
+    const long long n = a.n, c = blockIdx.x * 256ll + threadIdx.x;    // 2 n columns pass 32 bits
+    if (c >= n) return;
     float dw = 0.f, db = 0.f;
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float xh = (load_f32(a.x, row * a.ldx + c, a.x_type) - a.mean[row]) * a.rstd[row];
@@ -380,17 +386,17 @@ __global__ __launch_bounds__(256) void norm_grad_cols_kernel(const NormGradArgs 
         dw = __builtin_fmaf(g, xh, dw);
         db += g;
     }
-    float* out = a.partials + 2ll * blockIdx.y * a.n;
+    float* out = a.partials + 2 * blockIdx.y * n;
     out[c] = dw;
-    out[a.n + c] = db;
+    out[n + c] = db;
 }
 
 // Adds partial rows, 64 columns per workgroup: wave g of 16 adds rows g,
 // g + 16, ... in order, then the 16 sums meet in wave order.
-__global__ __launch_bounds__(1024) void partial_sum_kernel(const PartialSumArgs a) {
+__global__ __launch_bounds__(1024) void partial_sum_kernel(const PartialSumArgs a, long long first) {
     __shared__ float lds[16][64];
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const long long c = blockIdx.x * 64ll + lane;
+    const long long c = first + blockIdx.x * 64ll + lane;
     float s = 0.f;
     if (c < a.width) {
         int r = g;
@@ -504,7 +510,7 @@ hipError_t launch_norm_grad(const NormGradArgs& a, int cus, hipStream_t s) {
         trace_launch("norm_grad_long<%s>", a.x_type == kTypeF32 ? "fp32" : "bf16");
         st = hipGetLastError();
         if (st != hipSuccess || !sums) return st;
-        norm_grad_cols_kernel<<<dim3((a.n + 255) / 256, parts), 256, 0, s>>>(a);
+        norm_grad_cols_kernel<<<dim3((unsigned)((a.n + 255ll) / 256), parts), 256, 0, s>>>(a);
         trace_launch("norm_grad_cols");
         st = hipGetLastError();
     } else {
@@ -520,10 +526,15 @@ hipError_t launch_norm_grad(const NormGradArgs& a, int cus, hipStream_t s) {
 
 hipError_t launch_partial_sum(const PartialSumArgs& a, hipStream_t s) {
     const long long blocks = (a.width + 63) / 64;
-    if (blocks <= 0 || blocks > INT_MAX) return hipErrorInvalidValue;
-    partial_sum_kernel<<<(unsigned)blocks, 1024, 0, s>>>(a);
-    trace_launch("partial_sum");
-    return hipGetLastError();
+    if (blocks <= 0) return hipErrorInvalidValue;
+    constexpr long long kMost = (1 << 22) - 1;    // workgroups of a launch: its threads fit 32 bits
+    for (long long b = 0; b < blocks; b += kMost) {
+        partial_sum_kernel<<<(unsigned)std::min(blocks - b, kMost), 1024, 0, s>>>(a, 64 * b);
+        trace_launch("partial_sum");
+        const hipError_t st = hipGetLastError();
+        if (st != hipSuccess) return st;
+    }
+    return hipSuccess;
 }
 
 }  // namespace qg
