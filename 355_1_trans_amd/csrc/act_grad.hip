@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ActGradArgs a) {
             for (int e = 0; e < 8; ++e) {
                 // padding features have no dy: 0, whatever p holds there
                 const bool in = f + e < a.cols;
-                g[e] = in ? g[e] * (d[e] * u[e]) : 0.f;
+                g[e] = in ? through(a.act, g[e], d[e] * u[e]) : 0.f;
                 u[e] = in ? d[e] * y[e] : 0.f;
                 s0[e] += g[e];
                 s1[e] += u[e];
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ActGradArgs a) {
                 load8(a.pre + row * a.ldpre, n, a.n, g);
                 activate_slope<8>(a.act, g, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = f + e < a.cols ? d[e] * g[e] : 0.f;
+                for (int e = 0; e < 8; ++e) d[e] = f + e < a.cols ? through(a.act, g[e], d[e]) : 0.f;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) s0[e] += d[e];

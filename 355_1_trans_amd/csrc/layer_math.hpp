@@ -112,7 +112,7 @@ __device__ __forceinline__ void activate_slope(int act, float (&v)[E], float (&y
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             y[i] = v[i] < 0.f ? 0.f : v[i];
-            v[i] = v[i] > 0.f ? 1.f : 0.f;
+            v[i] = v[i] <= 0.f ? 0.f : 1.f;    // NaN is active, as in y
         }
         break;
     case kActSilu:
@@ -148,6 +148,11 @@ __device__ __forceinline__ void activate_slope(int act, float (&v)[E], float (&y
         }
         break;
     }
+}
+
+// dy act'(v) from the slope; relu passes dy on or stops it, also an infinite or NaN one
+__device__ __forceinline__ float through(int act, float slope, float dy) {
+    return act == kActRelu ? (slope != 0.f ? dy : 0.f) : slope * dy;
 }
 
 }  // namespace qg

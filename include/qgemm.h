@@ -297,6 +297,8 @@ size_t gemm_a4w4_mxfp4_gated_workspace_bytes(const opus_gemm_scale_kargs* args);
  *   linear  dp = dy * act'(p)          (pre unused for QGEMM_ACT_NONE)
  *   gated   dp = dg: dy * u * act'(g), du: dy * act(g), in w's row order
  *   dx = dp w,  dw = dp^T x,  dbias = sum over rows of dp
+ * (QGEMM_ACT_RELU: dp is dy, or dh u, where p > 0 or p is NaN, and 0 elsewhere,
+ * whatever dy holds there.)
  * dy [m, n] (gated: [m, features]), pre [m, n], x [m, k], w [n, k], dx [m, k]
  * and dw [n, k] are bf16, dbias [n] of dbias_dtype; each of dx, dw and dbias
  * may be NULL (with it w, or x).  Rows of x, w, dx and dw start on 16 bytes
