@@ -134,7 +134,8 @@ __device__ __forceinline__ void activate_slope(int act, float (&v)[E], float (&y
     case kActGeluTanh:
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float x2 = v[i] * v[i];
+            // bounded: past |v| = 1.8e19 the square would be infinite, and s (1 - s) = 0 times it NaN
+            const float x2 = fminf(v[i] * v[i], 1e30f);
             const float s = sigmoid(2.0f * kGeluC * v[i] * (1.0f + kGeluA * x2));
             y[i] = v[i] * s;
             v[i] = s + v[i] * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluA * x2);

@@ -43,3 +43,16 @@ def test_gated_relu_passes_or_stops(qgemm, gpu):
     dg, du = (t.float().tolist() for t in qgemm.split_gate_up(db, f))
     _same(dg, [0.0, 0.0, 15.0, INF, 8.0, 0.0])
     _same(du, [0.0, NAN, 10.0, 2.0, NAN, 0.0])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_largest_pre_activations(qgemm, gpu, act):
+    """Far from zero the slope is 1 or 0, up to the largest finite values."""
+    big = [1e4, 1e13, 1e19, 2e19, 1e30, 3e38]
+    _same(_dp(qgemm, gpu, act, big + [-v for v in big] + [0.0, 0.0], [2.0] * 14), [2.0] * 6 + [0.0] * 6 + [1.0] * 2)
+    n = len(big)
+    bias = torch.tensor(big + [-v for v in big] + [0.0, 0.0], device=gpu)       # A = 0: p is the bias
+    a, asc = qgemm.quant_mxfp8(torch.zeros((1, 128), device=gpu))
+    b, bsc = qgemm.quant_mxfp8(torch.ones((14, 128), device=gpu))
+    y = qgemm.linear_a8w8_mxfp8(a, b, asc, bsc, bias=bias, activation=act, dtype=torch.float32)[0]
+    assert torch.equal(y[:n], bias[:n]) and not y[n:].any()
