@@ -59,10 +59,16 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ActGradArgs a) {
             activate_slope<8>(a.act, g, y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                y[e] *= d[e];
+                d[e] *= u[e];
+            }
+            through<8>(a.act, g, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
                 // padding features have no dy: 0, whatever p holds there
                 const bool in = f + e < a.cols;
-                g[e] = in ? through(a.act, g[e], d[e] * u[e]) : 0.f;
-                u[e] = in ? d[e] * y[e] : 0.f;
+                g[e] = in ? d[e] : 0.f;
+                u[e] = in ? y[e] : 0.f;
                 s0[e] += g[e];
                 s1[e] += u[e];
             }
@@ -74,8 +80,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const ActGradArgs a) {
             if (a.act != kActNone) {
                 load8(a.pre + row * a.ldpre, n, a.n, g);
                 activate_slope<8>(a.act, g, y);
+                through<8>(a.act, g, d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = f + e < a.cols ? through(a.act, g[e], d[e]) : 0.f;
+                for (int e = 0; e < 8; ++e) d[e] = f + e < a.cols ? d[e] : 0.f;
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) s0[e] += d[e];

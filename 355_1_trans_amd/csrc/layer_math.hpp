@@ -157,9 +157,18 @@ __device__ __forceinline__ void activate_slope(int act, float (&v)[E], float (&y
     }
 }
 
-// dy act'(v) from the slope; relu passes dy on or stops it, also an infinite or NaN one
-__device__ __forceinline__ float through(int act, float slope, float dy) {
-    return act == kActRelu ? (slope != 0.f ? dy : 0.f) : slope * dy;
+// dy[i] act'(v[i]) from the slopes; relu passes dy on or stops it, also an infinite
+// or NaN one (a choice per element inside one loop for all activations cost 1 us of
+// a call's 125)
+template <int E>
+__device__ __forceinline__ void through(int act, const float (&slope)[E], float (&dy)[E]) {
+    if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) dy[i] = slope[i] != 0.f ? dy[i] : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) dy[i] *= slope[i];
+    }
 }
 
 }  // namespace qg
