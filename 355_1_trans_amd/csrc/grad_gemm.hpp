@@ -45,7 +45,7 @@ struct GradProduct {
     const uint16_t* b;       // [depth][ldb]
     uint16_t* c;             // bf16 [rows][ldc], rows on 16 bytes, cols a multiple of 8
     float* ws;               // splitk > 1: planes [splitk][rows][cols]
-    int rows, cols, depth;   // depth: a row-major A's padded row length
+    int rows, cols, depth;   // depth: the sum's length; a row-major A holds zeros from there to the next multiple of 64
     int tiles_m, tiles_n, group_m;
     int splitk, kt_per_split;
     int a_km;

@@ -425,11 +425,6 @@ bool aligned16(const void* p, long long ld, int elem) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem) % 16 == 0;
 }
 
-template <int T>
-constexpr int rows_per_block() {
-    return T == 64 ? 4 : 1;
-}
-
 // PER workgroups per CU walk the rows.  The threads of a row, its values per
 // thread and PER were timed over T = 64 - 1024, E = 8 - 32, PER = 1 - 8 at
 // M = 16384 bf16 (us): N = 7168 T 1024 E 8 PER 2 94.9, PER 1 108, 3 104, T 512
