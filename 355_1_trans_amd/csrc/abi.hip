@@ -1710,10 +1710,13 @@ hipError_t run_mx(const MxRoute& r, TileArgs t, const opus_gemm_scale_kargs& a, 
 // pick is 0.3 us slower at the median; the burst and band kernels it lacks gain
 // up to 2 us at N = 24576, K <= 4096.
 // With few K-tiles the 128 x 128 kernel takes over from the four-wave one, whose
-// single wave per SIMD has nothing to run beside its epilogue.  MXFP8 M = 5580,
-// N = 4836, gelu and residual (us, four-wave / 128 x 128): K = 256 86 / 44,
-// K = 1024 103 / 61, no activation 29 / 24 and 45 / 41; M = N = 8192 K = 256 114 /
-// 91 and 49 / 45, K = 1024 150 / 130 and 81 / 88.
+// single wave per SIMD has nothing to run beside its epilogue.  Six shapes (M = 1030 -
+// 16384, N = 2048 - 14336), 128 x 128 over four-wave time, geometric mean and the
+// slowest: up to 8 K-tiles MXFP8 plain 0.78 - 0.97 (1.04: M = 2048, N = 7168, K = 256
+// 14.4 us / 15.0), gated 0.84 - 0.96 (1.01), gelu and residual 0.66 - 0.74 (0.83); MXFP4
+// 0.81 - 0.92 (0.98), 0.82 - 0.94 (1.00), 0.64 - 0.73 (0.84).  Past 8 it depends on the
+// epilogue, which the route does not see: at 10 plain 1.10 (1.15) and 1.04 (1.11), gated
+// 1.09 (1.19) and 1.02 (1.08), gelu and residual still 0.81 and 0.79.
 // The kernel depends on the shape only, its K split on the workspace at hand.
 MxRoute route_mx_epi(const opus_gemm_scale_kargs& a, bool fp4, const WorkspaceView& w) {
     MxRoute r = route_mx(a, fp4, QGEMM_KID_AUTO, kAnyWorkspace);

@@ -191,9 +191,19 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void norm_kernel(const NormArgs 
 }
 
 // Rows past the registers: three passes over the row (the second and third
-// from cache), 1024 threads, one element at a time.  A thread's own sums, over
-// any number of elements, are in 64 bits.  n may be up to 2^31 - 1, which a
-// signed column counter would overflow on its way out of the loop.
+// from cache), 1024 threads, one element at a time.  M = 2048 bf16: N = 16400 68
+// us, N = 40000 204 (a pass over memory would be 56 at the copy's 5.9 TB/s); backward
+// 194 and 571.  A thread adds up to 64 elements in 32 bits and those sums in 64
+// (2^21 fp32 additions of one sign would lose 1e-3; 64 bits throughout took 1 - 5%
+// longer).  n may be up to 2^31 - 1, past which a signed column counter would go.
+template <class Body, class Flush>
+__device__ __forceinline__ void long_row(unsigned n, Body&& body, Flush&& flush) {
+    for (unsigned c0 = threadIdx.x; c0 < n; c0 += 64 * 1024) {
+        const unsigned end = min(n, c0 + 64 * 1024);
+        for (unsigned c = c0; c < end; c += 1024) body(c);
+        flush();
+    }
+}
 __global__ __launch_bounds__(1024) void norm_long_kernel(const NormArgs a) {
     __shared__ float lds[64];
     int half = 0;
@@ -202,15 +212,20 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const NormArgs a) {
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long x0 = row * a.ldx, y0 = row * a.ldy;
         double sum = 0.0;
-        for (unsigned c = threadIdx.x; c < n; c += 1024) sum += load_f32(a.x, x0 + c, a.x_type);
+        float part = 0.f;
+        const auto flush = [&]() __attribute__((always_inline)) {
+            sum += part;
+            part = 0.f;
+        };
+        long_row(n, [&](unsigned c) __attribute__((always_inline)) { part += load_f32(a.x, x0 + c, a.x_type); }, flush);
         float s[1] = {(float)sum};
         row_sums<1024, 1>(s, lds, half);
         const float mean = mean_of(s[0], len, inv);
         sum = 0.0;
-        for (unsigned c = threadIdx.x; c < n; c += 1024) {
-            const double d = load_f32(a.x, x0 + c, a.x_type) - mean;
-            sum += d * d;
-        }
+        long_row(n, [&](unsigned c) __attribute__((always_inline)) {
+            const float d = load_f32(a.x, x0 + c, a.x_type) - mean;
+            part = __builtin_fmaf(d, d, part);
+        }, flush);
         s[0] = (float)sum;
         row_sums<1024, 1>(s, lds, half);
         const float rstd = rsqrtf(__builtin_fmaf(s[0], inv, a.eps));
@@ -356,12 +371,17 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(const NormGradArgs
         const long long x0 = row * a.ldx, g0 = row * a.lddy, d0 = row * a.lddx;
         const float mean = a.mean[row], rstd = a.rstd[row];
         double sg = 0.0, sgx = 0.0;
-        for (unsigned c = threadIdx.x; c < n; c += 1024) {
+        float pg = 0.f, pgx = 0.f;
+        long_row(n, [&](unsigned c) __attribute__((always_inline)) {
             const float xh = (load_f32(a.x, x0 + c, a.x_type) - mean) * rstd;
             const float g = load_f32(a.dy, g0 + c, a.x_type) * (a.weight ? load_f32(a.weight, c, a.w_type) : 1.f);
-            sg += g;
-            sgx += (double)g * xh;
-        }
+            pg += g;
+            pgx = __builtin_fmaf(g, xh, pgx);
+        }, [&]() __attribute__((always_inline)) {
+            sg += pg;
+            sgx += pgx;
+            pg = pgx = 0.f;
+        });
         float s[2] = {(float)sg, (float)sgx};
         row_sums<1024, 2>(s, lds, half);
         const float c0 = s[0] * inv, c1 = s[1] * inv;

@@ -1,9 +1,9 @@
 """Layer norm of single rows whose column numbers, or twice them, pass 31 bits.
 
 Tolerances as in test_gpu_layer_norm.py: 32 x 2^-24 of the sizes that go into
-a value for its fp32 roundings (a thread's sums are in 64 bits, the 1024
-threads' are added in fp32 by wave, then 16 of them: 2^-24 of the sum of
-magnitudes for each of about ten levels), 2^-8 of the value for a bf16 output."""
+a value for its fp32 roundings (a thread adds 64 elements in fp32 and those
+sums in 64 bits; the 1024 threads' are added in fp32 by wave, then 16 of them:
+about ten levels), 2^-8 of the value for a bf16 output."""
 import pytest
 import torch
 
