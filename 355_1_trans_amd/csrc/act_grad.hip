@@ -7,6 +7,10 @@
 // 8 columns per lane (gated: 8 features, 16 columns), and walks every fourth
 // row of its workgroup's, so that column sums stay in registers; the four
 // waves' sums meet in LDS, in wave order.
+// The rounding to bf16 is the products' choice: fp32 operands have a sixteenth of
+// the bf16 matrix rate, and a second bf16 term of dp would double both products.
+// It moves dx and dw by 0.0015 of their norm (0.0023 off in all, their own rounding
+// 0.0017).  M = 2048, N = 4096: 12 us, 4.1 TB/s; gated, M = 4096, 2048 features: 19.
 #include <algorithm>
 
 #include "act_grad.hpp"

@@ -200,11 +200,12 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8], int lef
 // order), by one wave, bf16 out; EDGE: the columns may end inside the tile.  One loop for each activation, four rows at a time
 // without a branch between their LDS reads: with the general code below in their
 // place (every activation and edge case inside the row loop) an epilogue took
-// the time of its instruction fetches, ~15 us of a 256 x 256 tile's ~115
-// (MXFP8 M = 8192, N = 7168, K = 8192, no activation 397 -> 346 us, the product
-// without an epilogue 340; gelu 486 -> 379; gated 365 -> 356).  What a residual
-// adds (394) is its tile read by all CUs at once; touching its lines over the
-// last K-tiles instead slowed those by more (422).
+// the time of its instruction fetches, ~15 us of a 256 x 256 tile's ~115 (MXFP8 M =
+// 8192, N = 7168, K = 8192, no activation 397 us).  Now that is 348, the product
+// without an epilogue 340; with a bias 355, with gelu too 393, with a residual 385:
+// its tile is read by all CUs at once, and touching its lines over the last K-tiles
+// instead slowed those by more (422).  Gated, M = 4096, 8192 features, K = 7168: product
+// 326, silu 334, pre-activations saved too 355.
 template <int COLS, int ACT, bool EDGE>
 __device__ __forceinline__ void bf16_rows(const EpiArgs& e, const QG_LDS uint8_t* img, int L, int m0, int n0) {
     constexpr int U = 4;

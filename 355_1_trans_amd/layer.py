@@ -3,8 +3,10 @@ linear layers (bias, activation, residual) and gated feed-forward blocks on
 MXFP8 / MXFP4 operands, and their gradients.
 
 Calls launch on the current stream and record every tensor on it; there is no
-CPU fallback.  Sizes and row pitches (in elements) are below 2**31.  Gradients take the tensors that the forward call used and
-returned; nothing is kept between calls.
+CPU fallback.  Sizes and row pitches (in elements) are below 2**31.  The calls
+are not part of autograd: results carry no gradient, also where an input
+requires one, and the *_backward calls are made by hand, with the tensors that
+the forward call used and returned; nothing is kept between calls.
 """
 import ctypes
 
@@ -186,7 +188,7 @@ def linear_a8w8_mxfp8(A, B, A_scale, B_scale, bias=None, activation="none", resi
                       save_pre=False, out=None, workspace=None):
     """act(A B^T + bias) + residual in one pass: operands as gemm_a8w8_mxfp8 takes
     them; bias [N] and residual [M, N] fp32 or bf16; activation "none", "relu",
-    "silu", "gelu" (erf) or "gelu_tanh".  ``save_pre``: (y, A B^T + bias as
+    "silu", "gelu" (v Phi(v)) or "gelu_tanh".  ``save_pre``: (y, A B^T + bias as
     bf16), which linear_backward reads.  ``out`` may be the residual."""
     return _linear(False, A, B, A_scale, B_scale, bias, activation, residual, dtype, save_pre, out, workspace)
 

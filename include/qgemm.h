@@ -265,7 +265,7 @@ size_t gemm_a4w4_mxfp4_kid_workspace_bytes(const opus_gemm_scale_kargs* args, in
 #define QGEMM_ACT_NONE 0
 #define QGEMM_ACT_RELU 1
 #define QGEMM_ACT_SILU 2
-#define QGEMM_ACT_GELU 3         /* v Phi(v), by erf */
+#define QGEMM_ACT_GELU 3         /* v Phi(v); Phi within 1e-6 + v^2 2^-23 of itself */
 #define QGEMM_ACT_GELU_TANH 4    /* 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
 typedef struct qgemm_epilogue {
     const void* bias;        /* [n], or NULL */
